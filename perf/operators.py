@@ -15,7 +15,6 @@ Each case names the operator it measures ("op") and its sizes and types:
 With `own` false the plain form in elementary torch operations runs; with `own` true the calls of
 librfdetr.so.
 """
-import functools
 import math
 import random
 
@@ -350,9 +349,7 @@ def _plain(s):
 # ---- the library's calls ----------------------------------------------------
 
 
-@functools.lru_cache(maxsize=1)
 def _library():
-    """Loaded once, as a program does."""
     import os
     import sys
     package = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "rf-detr.cpp_b200")
