@@ -350,8 +350,12 @@ int rfdetr_b200_op_block_norm(const rfdetr_b200_block_norm* args, void* stream);
  * [tokens][kv_heads * head_dim], F16 or BF16, 16-byte aligned with pitches
  * that are multiples of 8; head h reads keys and values of head h / (heads /
  * kv_heads), at most 128 heads to one.  head_dim 64 or 128; max_len: at least
- * the longest length, and at most 2^25; 0 < scale <= 2e38.  The lengths stay
- * on the device.  A row whose every score is -infinity is NaN.  A NaN query or
+ * the longest length, and at most 2^25; 0 < scale <= 2e38, and scores
+ * (scale * q . k) of at most 2^26 in magnitude.  The lengths stay on the device.
+ * Scores, their maximum and the sum of the weights are f32; each weight is
+ * rounded to `type` for its product with v: off by at most 2^-8 (BF16) or
+ * 2^-11 (F16) of itself or, in F16, 2^-36 of the row's largest, so a result by
+ * that part of the weighted mean of |v| before its own rounding.  A row whose every score is -infinity is NaN.  A NaN query or
  * key reaches the rows that see it; an infinity or a NaN in v may also reach
  * rows of its sequence from which `causal` hides it (0 times infinity), as in
  * the plain form.  Neither reaches another sequence's rows. */

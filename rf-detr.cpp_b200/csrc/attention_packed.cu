@@ -15,8 +15,8 @@
 // the loads and first products of an item run while the last one's results leave.
 //   warps 0..3, 4..7  softmax of tile 0, 1: a thread owns a row, S from TMEM, exponentials in f32, P as
 //                     packed 16-bit pairs back to TMEM; the reference maximum is raised, and O in TMEM
-//                     rescaled, only when a row's maximum grows by more than 2^8 (numerator and
-//                     denominator share it)
+//                     rescaled, only when a row's maximum grows by more than 2^8, 2^4 in f16 (numerator
+//                     and denominator share it)
 //   warp 8            one lane issues tcgen05.mma: S_i = Q_i K^T and O_i += P_i V; while one tile's
 //                     softmax runs, the other tile's products do, and P V starts on the first 64 keys of
 //                     a block while the exponentials of the others are computed
@@ -43,7 +43,27 @@ namespace {
 
 constexpr int TQ = 128;               // rows of a tile
 constexpr int TK = 128;               // keys of a block
-constexpr float kRaise = 8.0f;        // growth of a row's maximum (log2) that moves its reference
+// The weights 2^(score - reference) enter the product with V as T, what the tensor core takes at its full rate (the error
+// against 64 bits grows from 1.5e-3 to 2.0e-3 in bf16, from 2.1e-4 to 2.7e-4 in f16, relative 2-norms on random inputs,
+// most of it the result's own rounding); the sums below them are those of the f32 weights.  The
+// reference is a row's maximum less LIFT, and moves when the maximum grows by more than RAISE (both log2).  bf16 rounds a
+// weight by at most 2^-8 of it, however small.  f16 does so down to 2^-14 and holds less in steps of 2^-24: with the
+// reference 2^11 below the maximum a weight is off by at most 2^-36 of its row's largest, and 2^25 of them, the most that a
+// row has, together by half a step of f16.  (Without it by 2^-25 each: 65535 weights of 2^-25.2, 1.7e-3 of the row, were 0.)
+// The largest weight is 2^(LIFT + RAISE) = 2^15; f16 ends at 2^16.
+template <typename T>
+struct Weights {
+    static constexpr bool HALF = __is_same(T, __half);
+    static constexpr float LIFT = HALF ? 11.0f : 0.0f, RAISE = HALF ? 4.0f : 8.0f;
+    // The reference of a maximum, and whether a row may keep its old one.  f16: rounded so that no weight is above
+    // 2^15, however far the scores' f32 spacing is above 1.
+    static __device__ __forceinline__ float reference(float top, float sl2) {
+        return HALF ? __fadd_ru(__fmul_ru(top, sl2), -LIFT) : top * sl2;
+    }
+    static __device__ __forceinline__ bool keeps(float old, float cand) {
+        return cand <= (HALF ? __fadd_rd(old, RAISE) : old + RAISE);
+    }
+};
 // Registers a thread: 384 threads are launched with 168; 128 x 88 + 256 x 208 = 384 x 168.
 constexpr int kLightRegs = 88, kSoftRegs = 208;
 
@@ -466,8 +486,9 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
 #pragma unroll
                     for (int e = 0; e < 32; ++e)
                         mx4[e & 3] = fmax3_nan(mx4[e & 3], __uint_as_float(r[h][e]), __uint_as_float(r[h + 1][e]));
-                const float m_cand = fmax3_nan(fmax3_nan(mx4[0], mx4[1], mx4[2]), mx4[3], -INFINITY) * sl2;
-                const float m_new = m_cand <= m + kRaise ? m : m_cand;  // the first finite one is always taken, and NaN
+                const float m_cand =
+                    Weights<T>::reference(fmax3_nan(fmax3_nan(mx4[0], mx4[1], mx4[2]), mx4[3], -INFINITY), sl2);
+                const float m_new = Weights<T>::keeps(m, m_cand) ? m : m_cand;  // the first finite one is always taken, and NaN
                 const float alpha = ex2(m - m_new);
                 if constexpr (C::APART) {
                     if (j > 0) {  // the previous product has read P, and O is at rest

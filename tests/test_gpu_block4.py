@@ -727,6 +727,46 @@ def test_attention_few_tiles(lens, heads, kv, d, causal):
     _attn(lens, heads, kv, d, causal, F16, seed=1, gain=3.0)
 
 
+@pytest.mark.parametrize("type", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("at", ["first", "last"])
+@pytest.mark.parametrize("n,weak", [(65536, -17.46875), (65536, -20.0), (131072, -23.0)])
+def test_attention_many_weak_keys(n, weak, at, d, type):
+    """One key of weight 1 and many of e^weak, too small for f16 beside it: together they are part of the row."""
+    t = mx_ref.TYPES[type]
+    q, k = torch.zeros(n, d, dtype=t, device=DEV), torch.zeros(n, d, dtype=t, device=DEV)
+    q[:, 0] = 1.0
+    k[:, 0] = weak
+    one = 0 if at == "first" else n - 1
+    k[one, 0] = 0.0
+    v = (1 + torch.rand(n, d, device=DEV, generator=_gen(n + d))).to(t)
+    v[one] = 0.0
+    o = _attention_once(q, k, v, d, type, 0, 1.0)
+    w = torch.exp(k[:, 0].double())
+    ref = (w @ v.double()) / w.sum()
+    # the roundings that _attn counts, with f16's weights within 2^-36 of the largest
+    u = mx_ref.half_step(t)
+    tol = (1.01 * u + 1e-5) * ref + u * ref + (n * 2.0 ** -36 * 2 + 2.0 ** -25 if t == torch.float16 else 0)
+    assert ref.min() > 2 * tol.max()
+    assert ((o.double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("type", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("n", [100, 700])
+def test_attention_equal_scores_of_great_size(n, sign, d, type):
+    """Scores of 2^25, some 3 apart where f32 holds them: the mean of the values."""
+    t = mx_ref.TYPES[type]
+    q = torch.full((n, d), 1024.0, dtype=t, device=DEV)
+    k = torch.full((n, d), sign * 32768.0 / d, dtype=t, device=DEV)
+    v = torch.randn(n, d, device=DEV, generator=_gen(d)).to(t)
+    o = _attention_once(q, k, v, d, type, 0, 1.0)
+    u = mx_ref.half_step(t)
+    mean, mag = v.double().mean(0), v.double().abs().mean(0)
+    assert ((o.double() - mean).abs() <= (1.01 * u + 1e-5) * mag + u * mean.abs() + 2.0 ** -25).all()
+
+
 def _attention_once(q, k, v, d, type, causal, scale):
     n = q.shape[0]
     o = torch.full((n, d), 7.0, dtype=q.dtype, device=DEV)
