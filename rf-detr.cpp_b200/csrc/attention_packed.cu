@@ -122,13 +122,13 @@ __device__ __forceinline__ int sequence_of_slot(const int32_t* cu, int n_seqs, i
     while (hi - lo > 31) {
         const int step = (hi - lo + 31) >> 5;
         const int s = lo + step * lane;
-        const bool below = s < hi && __ldg(cu + s) / span + s <= slot;
+        const bool below = s < hi && cu[s] / span + s <= slot;
         const int n = __popc(__ballot_sync(0xffffffffu, below));
         lo += step * (n > 0 ? n - 1 : 0);
         hi = min(hi, lo + step);
     }
     const int s = lo + lane;
-    const int c = s <= hi ? __ldg(cu + s) : 0;
+    const int c = s <= hi ? cu[s] : 0;
     const int n = __popc(__ballot_sync(0xffffffffu, s < hi && c / span + s <= slot));
     const int at = n > 0 ? n - 1 : 0;
     first = __shfl_sync(0xffffffffu, c, at);

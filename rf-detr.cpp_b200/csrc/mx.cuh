@@ -76,7 +76,9 @@ inline long long mx_pad_threads(int kt) { return 32ll * kt; }
 #ifdef __CUDACC__
 
 // The operators' kernels are launched while the stream's previous kernel still runs (where that lets them): each lets
-// the next start once its own CTAs have, and touches memory only behind the wait for all work before it.  Tensor memory
+// the next start once its own CTAs have, and touches memory only behind the wait for all work before it.  What earlier work
+// may have written changes while such a kernel is there already, so it is read by plain loads: neither __ldg nor __restrict__,
+// which let the compiler take the read-only path or move a load above the wait.  Tensor memory
 // is allocated behind the wait and before the next may start: a CTA that holds it never waits for one that needs it.
 __device__ __forceinline__ void wait_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }

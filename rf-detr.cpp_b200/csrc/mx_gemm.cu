@@ -389,7 +389,7 @@ k_mx_gemm(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
         auto fetch_bias = [&](int tile) {
             const int n = (tile % n_tiles) * BN + part * HC + lane;
 #pragma unroll
-            for (int c = 0; c < CH; ++c) next_bias[c] = n + 32 * c < p.N ? __ldg(p.bias + n + 32 * c) : 0.f;
+            for (int c = 0; c < CH; ++c) next_bias[c] = n + 32 * c < p.N ? p.bias[n + 32 * c] : 0.f;
         };
         if (p.bias && tile0 < num_tiles) fetch_bias(tile0);
         int local = 0;
@@ -628,7 +628,7 @@ k_mx_gemm_few(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
     if (warp >= 2 && ok && n < p.N) {  // a warp finishes a token, a lane four of its columns
         float b[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) b[i] = p.bias && n + i < p.N ? __ldg(p.bias + n + i) : 0.f;
+        for (int i = 0; i < 4; ++i) b[i] = p.bias && n + i < p.N ? p.bias[n + i] : 0.f;
         const uint32_t own_s = smem_u32(own + rank * held * BM + lane * 4), sums_s = smem_u32(sums + lane * 4);
         for (int c = warp - 2; c < mine; c += C::NEPI) {
             float x[4] = {};

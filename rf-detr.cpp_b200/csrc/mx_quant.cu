@@ -84,8 +84,8 @@ struct Ragged {
 // 16-byte aligned rows and k a multiple of 8.
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads)
-k_mx_quantize(const T* __restrict__ src, int ld, int k, uint8_t* __restrict__ codes, int ldc,
-              uint8_t* __restrict__ scales, int kt, const Units un, unsigned pad_from) {
+k_mx_quantize(const T* src, int ld, int k, uint8_t* codes, int ldc, uint8_t* scales, int kt,
+              const Units un, unsigned pad_from) {
     let_next_start();
     wait_previous();
     if (blockIdx.x >= pad_from) {
@@ -180,8 +180,8 @@ __device__ __forceinline__ void mx_values8(VecN<T, 8>& x, uint32_t w, uint32_t e
 
 template <typename T, bool VEC>
 __global__ void __launch_bounds__(kThreads)
-k_mx_dequantize(const uint8_t* __restrict__ codes, int ldc, const uint8_t* __restrict__ scales, int k,
-                T* __restrict__ dst, int ld, int kt, const Units un) {
+k_mx_dequantize(const uint8_t* codes, int ldc, const uint8_t* scales, int k, T* dst, int ld,
+                int kt, const Units un) {
     __shared__ __align__(16) typename Ragged<T, kBackUnit>::One buf[VEC ? 1 : kWarps][VEC ? 8 : kBackUnit];
     let_next_start();
     wait_previous();

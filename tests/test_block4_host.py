@@ -1,6 +1,8 @@
 """What the operators of a 4-bit transformer block refuse before any launch (no GPU needed: the
 pointers are addresses that nothing may touch), and the arithmetic of their plain 64-bit forms."""
 import ctypes as C
+import pathlib
+import re
 
 import pytest
 import torch
@@ -121,3 +123,17 @@ def test_reference_scale_tiles():
     assert t.numel() == lib.lib().rfdetr_b200_mx_scale_bytes(130, 5 * 32)
     assert t[(1 * 2 + 1) * 512 + 1 * 16 + 0 * 4 + 0] == s[129, 4]
     assert t[(0 * 2 + 0) * 512 + 5 * 16 + 2 * 4 + 3] == s[69, 3]
+
+
+@pytest.mark.parametrize("name", ["mx.cuh", "mx_quant.cu", "mx_gemm.cu", "block_norm.cu", "attention_packed.cu"])
+def test_kernels_that_start_early_read_memory_by_plain_loads(name):
+    """These kernels are there while earlier ones still write what they will read, so nothing they read may be
+    declared constant for their lifetime: no read-only loads, no pointers that promise it to the compiler."""
+    source = (pathlib.Path(lib.__file__).parents[1] / "csrc" / name).read_text()
+    code = re.sub(r"//[^\n]*", "", source)
+    for word in ("__ldg", "__restrict", "ld.global.nc"):
+        assert word not in code, word
+    if name != "mx.cuh":
+        assert "launch_early(" in code
+        # every kernel waits for the work before it
+        assert len(re.findall(r"\bwait_previous\(\)", code)) == len(re.findall(r"__global__", code)) > 0
