@@ -560,8 +560,10 @@ k_mx_gemm_few(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
         if (elect_one()) {
             int s = 0;
             uint32_t phase = 0;
+            bool all = true;
             for (int kb = kb0; kb < kb1; ++kb) {
-                if (!mbar_wait(&full[s], phase, cta_abort, nullptr)) break;
+                all = mbar_wait(&full[s], phase, cta_abort, nullptr);
+                if (!all) break;
                 tc_fence_after();
                 const uint32_t b0 = smem_u32(sB + s * C::B_BYTES), a0 = smem_u32(sA + s * C::A_BYTES);
                 const uint32_t sf0 = smem_u32(sSF + s * 2 * SF_GROUP);
@@ -584,7 +586,7 @@ k_mx_gemm_few(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
                     phase ^= 1;
                 }
             }
-            umma_commit(done);
+            if (all) umma_commit(done);  // else nobody takes the sums for whole
         }
     }
     const int quad = warp & 3, row = quad * 32 + lane;

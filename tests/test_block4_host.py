@@ -137,3 +137,22 @@ def test_kernels_that_start_early_read_memory_by_plain_loads(name):
         assert "launch_early(" in code
         # every kernel waits for the work before it
         assert len(re.findall(r"\bwait_previous\(\)", code)) == len(re.findall(r"__global__", code)) > 0
+
+
+def _kernel(name, kernel):
+    """The text of a kernel in csrc/, comments left out."""
+    source = (pathlib.Path(lib.__file__).parents[1] / "csrc" / name).read_text()
+    code = re.sub(r"//[^\n]*", "", source)
+    at = code.index(kernel + "(")
+    return code[at:code.index("\n}\n", at)]
+
+
+def test_split_product_sums_are_whole_or_not_announced():
+    """The issuing warp tells the epilogue that the sums are there (a commit to `done`, once) only where no wait
+    for a stage ran out: the loop over the stages keeps what each wait said, and the commit asks for it."""
+    code = _kernel("mx_gemm.cu", "k_mx_gemm_few")
+    assert code.count("umma_commit(done)") == 1
+    guard = re.search(r"if \((\w+)\) umma_commit\(done\)", code)
+    assert guard
+    kept = guard.group(1)
+    assert re.search(kept + r" = mbar_wait\(&full\[s\], phase, cta_abort, [^;]*;\s*if \(!" + kept + r"\) break;", code)
