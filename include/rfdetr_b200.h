@@ -276,6 +276,11 @@ int rfdetr_b200_op_conv3x3_noalloc(const void* src, int lds, int batch, int h, i
  * described here are refused with cudaErrorInvalidValue before any launch;
  * a call with no rows or tokens succeeds and does nothing.
  *
+ * Inside, the product and the attention wait for their own copies and products,
+ * each wait for two seconds at most (they take microseconds).  One that runs out
+ * leaves the call's result incomplete and the device's error word non-zero: see
+ * rfdetr_b200_op_error_word.
+ *
  * Microscaled operand (MXFP4): a matrix [rows][k] as
  *   codes   E2M1 values, two to a byte (the even column in the low nibble),
  *           row r at codes + r * ld_codes, ceil(k / 32) * 16 bytes of it, zeros
@@ -292,6 +297,13 @@ int rfdetr_b200_op_conv3x3_noalloc(const void* src, int lds, int batch, int h, i
  * code), at most 6 in magnitude.  A block that holds an infinity or a NaN
  * gets the scale NaN, so that everything computed from it is NaN. */
 size_t rfdetr_b200_mx_scale_bytes(int rows, int k);
+
+/* Device address of the current device's error word, an int that is 0 until a
+ * wait in a kernel of these operators runs out, on any stream; the first such
+ * code stays.  Results computed before the word was read as 0, behind them on
+ * their stream (an asynchronous copy of 4 bytes, which may be captured), are
+ * complete.  The caller sets it back to 0. */
+int rfdetr_b200_op_error_word(int** word);
 
 /* src [rows][ld] of `type` -> microscaled operand of [rows][k]. */
 int rfdetr_b200_op_mx_quantize(const void* src, int type, int ld, int rows, int k, void* codes, int ld_codes,

@@ -73,6 +73,7 @@ struct PackedArgs {
     int n_seqs, tokens, ldo, kv_heads, group, tt, tiles, causal;
     int by_keys;  // the two softmax halves of a CTA share one tile's keys, not two tiles
     float sl2;  // scale / ln 2
+    int* err;   // the device's error word, set by a wait that runs out
 };
 
 // What a CTA works on: rows [t0, t0 + tiles * tt) of the sequence whose tokens start at `start`.
@@ -607,6 +608,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
     }
     tc_fence_before();
     __syncthreads();
+    report_abort(cta_abort, p.err);
     if (warp == 8) {
         tc_fence_after();
         tmem_dealloc(tmem, 512);
@@ -631,6 +633,7 @@ cudaError_t launch(const void* q, const void* k, const void* v, int ldq, int ldk
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e == cudaSuccess) e = op_error_word(dev, &p.err);
     if (e != cudaSuccess) return e;
     const uint64_t bit = 1ull << (dev & 63);
     if (!(attr.load() & bit)) {
@@ -680,7 +683,7 @@ cudaError_t attention_packed(const void* q, const void* k, const void* v, int ld
     if (!cu_seqlens || !ptr_aligned(cu_seqlens, 4)) return cudaErrorInvalidValue;
     if (!tensor_map_encode()) return cudaErrorNotSupported;
     const PackedArgs p = {o, cu_seqlens, n_seqs, tokens, ldo, kv_heads, heads / kv_heads, 0, 0, causal != 0, 0,
-                          scale * 1.4426950408889634f};
+                          scale * 1.4426950408889634f, nullptr};
     if (type == MX_F16)
         return head_dim == 64 ? launch<__half, 64>(q, k, v, ldq, ldk, ldv, p, max_len, st)
                               : launch<__half, 128>(q, k, v, ldq, ldk, ldv, p, max_len, st);

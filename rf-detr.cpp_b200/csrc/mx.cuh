@@ -51,6 +51,9 @@ inline PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encode() {
     return fn;
 }
 
+// The error word of device `dev`, the current one: 0 until a kernel's wait runs out (sm100.cuh).
+cudaError_t op_error_word(int dev, int** word);
+
 cudaError_t mx_quantize(const void* src, int type, int ld, int rows, int k, uint8_t* codes, int ldc, uint8_t* scales,
                         cudaStream_t st);
 cudaError_t mx_dequantize(const uint8_t* codes, int ldc, const uint8_t* scales, int rows, int k, void* dst, int type,

@@ -42,6 +42,7 @@ struct MxArgs {
     int tma_out;       // the output leaves by TMA, or
     int row_boundary;  // bytes on whose boundaries all its rows lie: 8, 4 or 2
     int vec_out;  // its rows on boundaries of four elements
+    int* err;     // the device's error word, set by a wait that runs out
 };
 
 template <int BN, bool CTA2>
@@ -449,6 +450,7 @@ k_mx_gemm(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
     tc_fence_before();
     if constexpr (CTA2) cluster_sync();  // the peer may still arrive here, and the pair frees its TMEM together
     else __syncthreads();
+    report_abort(cta_abort, p.err);
     if (warp == 1) {
         tc_fence_after();
         if constexpr (CTA2) tmem_dealloc_pair(tmem, C::TMEM_COLS);
@@ -662,6 +664,7 @@ k_mx_gemm_few(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
     if (parts > 1) cluster_sync();  // nobody still reads or writes another's shared memory
     tc_fence_before();
     __syncthreads();
+    report_abort(cta_abort, p.err);
     if (warp == 1) {
         tc_fence_after();
         tmem_dealloc(tmem, C::TMEM_COLS);
@@ -772,10 +775,11 @@ cudaError_t launch_few(const MxOperands& o, MxArgs p, int dev, int sms, cudaStre
 }
 
 template <typename T>
-cudaError_t dispatch(const MxOperands& o, const MxArgs& p, cudaStream_t st) {
+cudaError_t dispatch(const MxOperands& o, MxArgs p, cudaStream_t st) {
     int dev = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&dev);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    if (e == cudaSuccess) e = op_error_word(dev, &p.err);
     if (e != cudaSuccess) return e;
     // A stage takes a CTA about 0.25 us; bringing the parts of TN tokens together 0.8 (32) to 4 us (128).  So K
     // is split where that saves TN / 8 stages or more: 1 x 4096 of K = 4096 5.3 us against 7.7, 32 x 4096 of
@@ -814,7 +818,7 @@ cudaError_t mx_gemm(const uint8_t* a, int lda, const uint8_t* a_scales, const ui
         return cudaErrorInvalidValue;
     if (!tensor_map_encode()) return cudaErrorNotSupported;
     const MxOperands o = {a, a_scales, b, b_scales, lda, ldb};
-    const MxArgs p = {M, N, K, ldo, act, bias, out, 0, 0, 0};
+    const MxArgs p = {M, N, K, ldo, act, bias, out, 0, 0, 0, nullptr};
     switch (out_type) {
         case MX_F32: return dispatch<float>(o, p, st);
         case MX_F16: return dispatch<__half>(o, p, st);

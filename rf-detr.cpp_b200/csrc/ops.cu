@@ -9,6 +9,30 @@
 #include "quant.cuh"
 #include "select.cuh"
 
+#include <atomic>
+
+namespace rfb {
+
+namespace {
+__device__ int g_op_error;
+}
+
+cudaError_t op_error_word(int dev, int** word) {
+    static std::atomic<int*> known[64];  // its address on a device never changes
+    if (dev < 64 && (*word = known[dev].load())) return cudaSuccess;
+    void* p = nullptr;
+    const cudaError_t e = cudaGetSymbolAddress(&p, g_op_error);
+    if (e != cudaSuccess) {
+        cudaGetLastError();
+        return e;
+    }
+    *word = static_cast<int*>(p);
+    if (dev < 64) known[dev].store(*word);
+    return cudaSuccess;
+}
+
+}  // namespace rfb
+
 extern "C" int rfdetr_b200_op_gemm(const void* A, int lda, const void* B, int ldb, int M, int N, int K, int epi,
                                    int act, const float* bias, const float* colscale, const float* ln_g,
                                    const float* ln_b, float ln_eps, const float* resid, int ldr, float* out32,
@@ -146,6 +170,14 @@ extern "C" int rfdetr_b200_op_conv3x3(const void* src, int lds, int batch, int h
     a.out32 = out32; a.ld32 = ld32;
     a.out16 = static_cast<__half*>(out16); a.ld16 = ld16;
     return (int)rfb::gemm(a, st);
+}
+
+extern "C" int rfdetr_b200_op_error_word(int** word) {
+    if (!word) return (int)cudaErrorInvalidValue;
+    *word = nullptr;
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    return (int)(e == cudaSuccess ? rfb::op_error_word(dev, word) : e);
 }
 
 extern "C" size_t rfdetr_b200_mx_scale_bytes(int rows, int k) {

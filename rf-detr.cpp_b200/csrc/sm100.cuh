@@ -107,6 +107,12 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volati
     }
 }
 
+// Behind the CTA's last barrier: tells the host that a wait of this CTA ran out.  (One place for all waits: an error word
+// in each costs the roles registers.)
+__device__ __forceinline__ void report_abort(const volatile int* cta_abort, int* err) {
+    if (threadIdx.x == 0 && *cta_abort) atomicCAS(err, 0, kErrWaitTimeout);
+}
+
 // 3-D tiled TMA load global -> shared, completing on `bar` (complete_tx).
 __device__ __forceinline__ void tma_load_3d(const CUtensorMap* map, uint64_t* bar, void* dst, int x, int y, int z) {
     asm volatile(

@@ -151,6 +151,7 @@ SIGNATURES = {
     "rfdetr_b200_op_conv3x3_noalloc": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_int,
                                                  C.c_void_p, C.c_int, C.c_void_p, C.c_void_p, C.c_float, C.c_int,
                                                  C.c_void_p, C.c_int, C.c_void_p, C.c_int, C.c_void_p]),
+    "rfdetr_b200_op_error_word": (C.c_int, [C.POINTER(C.c_void_p)]),
     "rfdetr_b200_mx_scale_bytes": (C.c_size_t, [C.c_int, C.c_int]),
     "rfdetr_b200_op_mx_quantize": (C.c_int, [C.c_void_p, C.c_int, C.c_int, C.c_int, C.c_int, C.c_void_p, C.c_int,
                                              C.c_void_p, C.c_void_p]),

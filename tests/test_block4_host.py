@@ -156,3 +156,18 @@ def test_split_product_sums_are_whole_or_not_announced():
     assert guard
     kept = guard.group(1)
     assert re.search(kept + r" = mbar_wait\(&full\[s\], phase, cta_abort, [^;]*;\s*if \(!" + kept + r"\) break;", code)
+
+
+@pytest.mark.parametrize("name,kernel", [("mx_gemm.cu", "k_mx_gemm"), ("mx_gemm.cu", "k_mx_gemm_few"),
+                                         ("attention_packed.cu", "k_attn_packed")])
+def test_a_wait_that_runs_out_is_reported(name, kernel):
+    """Every bounded wait sets the CTA's word, and behind the CTA's last barrier that word goes to the device's."""
+    code = _kernel(name, kernel)
+    waits = re.findall(r"\bmbar_wait(?:<\w+>)?\([^;]*?, cta_abort, nullptr\)", code)
+    assert len(waits) == len(re.findall(r"\bmbar_wait\b", code)) >= 4
+    assert len(re.findall(r"__syncthreads\(\);\s*report_abort\(cta_abort, p\.err\);", code)) == 1
+    assert "__syncthreads" not in code[code.index("report_abort"):] and "return;" not in code
+
+
+def test_error_word_refusal():
+    assert lib.lib().rfdetr_b200_op_error_word(None) == INVALID

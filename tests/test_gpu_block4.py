@@ -1,6 +1,12 @@
 """The operators of a 4-bit transformer block on the B200 against their plain forms in 64 bits:
 microscaled quantisation and product, block norms, attention over packed sequences."""
+import ctypes as C
 import math
+import os
+import pathlib
+import shutil
+import subprocess
+import sys
 
 import pytest
 import torch
@@ -1110,3 +1116,105 @@ def test_captured_with_copies_and_a_second_stream_between():
         codes, e = mx_ref.quantize(total.double())
         assert torch.equal(bufs[0][0], mx_ref.pack(codes)) and torch.equal(bufs[0][1], mx_ref.tile_scales(e))
         assert torch.equal(total, (bufs[0][2] + bufs[1][2]).bfloat16())
+
+
+# ---- waits that run out -----------------------------------------------------------------
+
+WAIT_PROBE = r"""
+#include "sm100.cuh"
+// A wait for an arrival that nobody makes, and the word that it leaves.
+__global__ void k_wait(int* err) {
+    __shared__ uint64_t bar;
+    __shared__ int cta_abort;
+    if (threadIdx.x == 0) {
+        rfb::mbar_init(&bar, 1);
+        cta_abort = 0;
+        rfb::fence_mbar_init();
+        rfb::mbar_wait(&bar, 0, &cta_abort, nullptr);
+    }
+    __syncthreads();
+    rfb::report_abort(&cta_abort, err);
+}
+extern "C" int wait_for_nothing(int* err, void* stream) {
+    k_wait<<<1, 32, 0, static_cast<cudaStream_t>(stream)>>>(err);
+    return (int)cudaGetLastError();
+}
+"""
+
+
+def _error_word():
+    word = C.c_void_p()
+    assert _lib().rfdetr_b200_op_error_word(C.byref(word)) == 0 and word.value
+    return word.value
+
+
+class _DeviceInt:
+    """Device memory at an address as torch sees it."""
+
+    def __init__(self, at):
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (at, False), "version": 2}
+
+
+def test_error_word_stays_zero():
+    """The calls of this file leave it alone; it is the same address every time."""
+    at = _error_word()
+    assert at == _error_word()
+    word = torch.as_tensor(_DeviceInt(at), device=DEV)
+    _gemm(300, 300, 16384, 0, BF16, False)
+    _attn([700, 3], 4, 2, 64, True, BF16)
+    assert word.item() == 0
+
+
+def test_a_wait_that_runs_out_sets_the_error_word(tmp_path):
+    """The operators' bounded wait, in a kernel of its own, for an arrival that nobody makes: it returns after its
+    two seconds, the context lives on, the word tells, and the caller clears it."""
+    nvcc = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
+    if not os.path.exists(nvcc):
+        pytest.skip("no nvcc")
+    (tmp_path / "probe.cu").write_text(WAIT_PROBE)
+    csrc = pathlib.Path(__file__).parents[1] / "rf-detr.cpp_b200" / "csrc"
+    subprocess.run([nvcc, "-gencode", "arch=compute_100a,code=sm_100a", "-std=c++17", "-O2", "-shared", "-Xcompiler", "-fPIC",
+                    "-cudart", "shared", "-I", str(csrc), "-o", str(tmp_path / "probe.so"), str(tmp_path / "probe.cu")],
+                   check=True)
+    probe = C.CDLL(str(tmp_path / "probe.so")).wait_for_nothing
+    probe.argtypes = [C.c_void_p, C.c_void_p]
+    at = _error_word()
+    word = torch.as_tensor(_DeviceInt(at), device=DEV)
+    assert word.item() == 0
+    assert probe(at, _stream()) == 0
+    # calls behind it run, and neither clear the word nor set it anew
+    _gemm(70, 64, 512, 0, BF16, False)
+    code = word.item()
+    assert code & 0xff == 1
+    _attn([200], 2, 1, 128, True, BF16)
+    assert word.item() == code
+    word.zero_()
+    _gemm(70, 64, 512, 0, BF16, False)
+    assert word.item() == 0
+
+
+def test_first_call_of_a_process_may_be_captured():
+    """Nothing that a first call sets up keeps it from being captured."""
+    code = """
+import sys, torch
+sys.path[:0] = [%r, %r]
+import mx_ref, test_gpu_block4 as t
+g = t._gen(0)
+(a, sa, A), (b, sb, B) = t._operand(g, 70, 512), t._operand(g, 64, 512)
+x = torch.randn(200, 192, device=t.DEV, generator=g).bfloat16()
+cu = torch.tensor([0, 200], dtype=torch.int32, device=t.DEV)
+y, o = torch.zeros(70, 64, device=t.DEV), torch.zeros(200, 64, device=t.DEV).bfloat16()
+graph = torch.cuda.CUDAGraph()
+torch.cuda.synchronize()
+with torch.cuda.graph(graph):
+    st = torch.cuda.current_stream().cuda_stream
+    L = t._lib()
+    assert L.rfdetr_b200_op_mx_gemm(t._p(a), 256, t._p(sa), t._p(b), 256, t._p(sb), 70, 64, 512, 0, None, t._p(y), 0, 64, st) == 0
+    assert L.rfdetr_b200_op_attention_packed(t._p(x), t._p(x[:, 64:]), t._p(x[:, 128:]), 192, 192, 192, t._p(o), 64, 30, t._p(cu),
+                                             1, 200, 200, 1, 1, 64, 1, 0.125, st) == 0
+graph.replay()
+torch.cuda.synchronize()
+assert ((y.double() - A @ B.T).abs() <= t._gemm_tolerance(A, B, A @ B.T, torch.float32, 0, None)).all()
+assert torch.isfinite(o.float()).all() and (o[0] == x[0, 128:]).all()
+""" % (str(pathlib.Path(__file__).parent), str(pathlib.Path(__file__).parents[1] / "rf-detr.cpp_b200"))
+    subprocess.run([sys.executable, "-c", code], check=True, timeout=300)
