@@ -397,6 +397,123 @@ def test_gemm_is_deterministic(M, N, K):
         assert torch.equal(first, _gemm(M, N, K, 0, F32, True))
 
 
+# Shapes that a B200's 148 SMs take with the 256 columns wide tiles: at least 148 tiles of 128 x 256; with pairs of SMs from
+# K = 2048 (4096 with GELU or SiLU) where these need no more turns.  Odd numbers of row tiles, rows and columns that end
+# inside a tile, K that ends inside a stage.
+WIDE = [(2400, 2051, 600), (4097, 2048, 512), (2433, 2304, 1000)]
+PAIRS = [(2400, 2051, 2050), (2433, 2304, 4128), (4100, 1300, 4500)]
+
+
+@pytest.mark.parametrize("type", [F32, F16, BF16])
+@pytest.mark.parametrize("act", [0, 1, 2, 3])
+@pytest.mark.parametrize("M,N,K", WIDE + PAIRS)
+def test_gemm_wide_tiles(M, N, K, act, type):
+    _gemm(M, N, K, act, type, True)
+    _gemm(M, N, K, act, type, False, ldo=N + 5)
+
+
+@pytest.mark.parametrize("type", [F32, F16, BF16])
+@pytest.mark.parametrize("M,N,K", [WIDE[0], PAIRS[0]])
+def test_gemm_wide_tiles_every_output_alignment(M, N, K, type):
+    """As test_gemm_every_output_alignment."""
+    t = mx_ref.TYPES[type]
+    g = _gen(M)
+    a, sa, A = _operand(g, M, K)
+    b, sb, B = _operand(g, N, K)
+    ref = A @ B.T
+    tol = _gemm_tolerance(A, B, ref, t, 0, None)
+    for pad, offset in ((0, 0), (5, 0), (5, 1), (1, 0), (3, 2), (13, 8), (0, 1)):
+        out = torch.full((M * (N + pad) + 32,), 7.0, dtype=t, device=DEV)
+        assert _lib().rfdetr_b200_op_mx_gemm(_p(a), a.shape[1], _p(sa), _p(b), b.shape[1], _p(sb), M, N, K, 0, None,
+                                             out[offset:].data_ptr(), type, N + pad, _stream()) == 0
+        got = torch.as_strided(out, (M, N), (N + pad, 1), offset)
+        assert ((got.double() - ref).abs() <= tol).all()
+        got.fill_(7.0)
+        assert (out == 7.0).all()
+
+
+@pytest.mark.parametrize("act", [0, 1, 2, 3])
+@pytest.mark.parametrize("M,N,K", [WIDE[0], PAIRS[0], PAIRS[1]])
+def test_gemm_wide_tiles_nan(M, N, K, act):
+    """Rows with a NaN scale and a column with a NaN bias, in every column chunk's epilogue; none but these."""
+    g = _gen(M)
+    a, sa, A = _operand(g, M, K)
+    b, sb, B = _operand(g, N, K)
+    rows = [0, 127, 128, 1000, M - 1]
+    e = torch.full((M, -(-K // 32)), 127, dtype=torch.uint8, device=DEV)
+    e[rows, 3] = 255
+    bias = torch.zeros(N, device=DEV)
+    bias[[5, 255, 256, 1023, N - 1]] = math.nan
+    out = torch.zeros(M, N, dtype=torch.bfloat16, device=DEV)
+    assert _lib().rfdetr_b200_op_mx_gemm(_p(a), a.shape[1], _p(mx_ref.tile_scales(e)), _p(b), b.shape[1], _p(sb), M, N, K, act,
+                                         _p(bias), _p(out), BF16, N, _stream()) == 0
+    nan = torch.isnan(bias)[None].repeat(M, 1)
+    nan[rows] = True
+    assert torch.equal(torch.isnan(out), nan)
+
+
+def _exact_operand(g, rows, k):
+    """Any codes, scales 1/2, 1 and 2: multiples of 1/4 up to 12, whose products' sums are exact in f32 while the
+    sum of their magnitudes is below 2^24 / 16."""
+    codes = torch.randint(0, 16, (rows, k), device=DEV, generator=g).to(torch.uint8)
+    codes = torch.nn.functional.pad(codes, (0, -k % 32))
+    e = torch.randint(126, 129, (rows, -(-k // 32)), device=DEV, generator=g).to(torch.uint8)
+    return mx_ref.pack(codes).contiguous(), mx_ref.tile_scales(e), mx_ref.values(codes, e)
+
+
+EXACT = [(1, 4096, 4096), (1, 130, 16384), (13, 11008, 4096), (16, 500, 8192), (30, 300, 8192), (61, 131, 16384),
+         (64, 256, 16384), (150, 131, 16384), (300, 300, 16384), (500, 500, 8200), (200, 700, 1000), (1616, 1152, 384),
+         (2400, 2051, 600), (2400, 2051, 2050), (2433, 2304, 8192)]
+
+
+@pytest.mark.parametrize("M,N,K", EXACT)
+def test_gemm_exact_sums(M, N, K):
+    """Products whose sums f32 holds exactly in any order: the results are those of 64 bits, rounded once, so a
+    block with another's scale, a stage twice or not at all, or a part of K that is missing shows."""
+    g = _gen(M + K)
+    a, sa, A = _exact_operand(g, M, K)
+    b, sb, B = _exact_operand(g, N, K)
+    bias = torch.randint(-40, 40, (N,), device=DEV, generator=g).float()
+    ref = A @ B.T
+    assert (A.abs() @ B.abs().T).max() + 40 < 2 ** 20
+    for type, bi in ((F32, None), (F32, bias), (BF16, bias), (F16, None)):
+        t = mx_ref.TYPES[type]
+        out = torch.full((M, N), 7.0, dtype=t, device=DEV)
+        assert _lib().rfdetr_b200_op_mx_gemm(_p(a), a.shape[1], _p(sa), _p(b), b.shape[1], _p(sb), M, N, K, 0, _p(bi), _p(out),
+                                             type, N, _stream()) == 0
+        assert torch.equal(out, (ref + bi.double() if bi is not None else ref).to(t))
+
+
+@pytest.mark.parametrize("M,N,K", EXACT)
+def test_gemm_one_block_of_each_row(M, N, K):
+    """Rows of A with one block that is not zero, another for each row: every block of K counts once, with its own
+    scales."""
+    g = _gen(M + K + 1)
+    kb = -(-K // 32)
+    codes = torch.randint(0, 16, (M, kb, 32), device=DEV, generator=g).to(torch.uint8)
+    b, sb, B = _exact_operand(g, N, K)
+    for first in range(0, kb, max(M, kb // 32)):  # one row at a time: 32 of the blocks
+        at = (first + torch.arange(M, device=DEV)) % kb
+        here = torch.zeros(M, kb, dtype=torch.bool, device=DEV)
+        here[torch.arange(M, device=DEV), at] = True
+        c = torch.where(here[..., None], codes, torch.zeros_like(codes)).view(M, -1)
+        c = torch.where(torch.arange(c.shape[1], device=DEV) < K, c, torch.zeros_like(c))
+        e = torch.randint(126, 129, (M, kb), device=DEV, generator=g).to(torch.uint8)
+        A = mx_ref.values(c, e)
+        out = torch.full((M, N), 7.0, device=DEV)
+        a, sa = mx_ref.pack(c).contiguous(), mx_ref.tile_scales(e)
+        assert _lib().rfdetr_b200_op_mx_gemm(_p(a), a.shape[1], _p(sa), _p(b), b.shape[1], _p(sb), M, N, K, 0, None, _p(out),
+                                             F32, N, _stream()) == 0
+        assert torch.equal(out.double(), A @ B.T)
+
+
+@pytest.mark.parametrize("M,N,K", [(2400, 2051, 600), (2400, 2051, 2050)])
+def test_gemm_wide_tiles_are_deterministic(M, N, K):
+    first = _gemm(M, N, K, 1, F32, True)
+    for _ in range(3):
+        assert torch.equal(first, _gemm(M, N, K, 1, F32, True))
+
+
 # ---- norms ------------------------------------------------------------------------
 
 
