@@ -948,6 +948,143 @@ def test_attention_weight_of_unseen_keys_is_zero(d):
     assert (o[0] == 0).all()
 
 
+# Heads of one sequence that a B200's 148 SMs take as single tiles whose keys are shared out, and so many that a CTA has
+# two tiles.
+FEW_OR_MANY = [1, 160]
+
+
+def _attention_same_heads(q, k, v, heads, type, causal, scale, lens=None):
+    """The same q, k and v [tokens][d] for every head, each with keys of its own; every head's result is the same."""
+    n, d = q.shape
+    lens = lens or [n]
+    q, k, v = (x.repeat(1, heads) for x in (q, k, v))
+    o = torch.full((n, heads * d), 7.0, dtype=q.dtype, device=DEV)
+    cu = torch.tensor([sum(lens[:i]) for i in range(len(lens) + 1)], dtype=torch.int32, device=DEV)
+    assert _lib().rfdetr_b200_op_attention_packed(_p(q), _p(k), _p(v), heads * d, heads * d, heads * d, _p(o), heads * d, type,
+                                                  _p(cu), len(lens), n, max(lens), heads, heads, d, int(causal), scale,
+                                                  _stream()) == 0
+    bits = o.view(n, heads, d)
+    assert torch.equal(bits.isnan(), bits[:, :1].isnan().expand_as(bits))
+    assert torch.equal(bits.nan_to_num(), bits[:, :1].nan_to_num().expand_as(bits))
+    return o[:, :d]
+
+
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("lens,heads,kv", [([520], 160, 160), ([700, 130, 1, 0, 257], 80, 80), ([1100, 900], 128, 32),
+                                           ([300, 385], 224, 32), ([129] * 40, 40, 10)])
+def test_attention_two_tiles(lens, heads, kv, d, causal):
+    """So many tiles that a CTA takes two of a sequence: both full, the second short or not there, one item or more
+    after another."""
+    _attn(lens, heads, kv, d, causal, BF16, behind=5)
+    _attn(lens, heads, kv, d, causal, F16, seed=1, gain=3.0)
+
+
+@pytest.mark.parametrize("heads", FEW_OR_MANY)
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("type", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n", [100, 300, 700])
+def test_attention_equal_scores_running_mean(n, d, type, causal, heads):
+    """Keys that are all zero: the mean of the values up to each position, or of all, which differ from row to row."""
+    t = mx_ref.TYPES[type]
+    q, k = torch.randn(n, d, device=DEV, generator=_gen(0)).to(t), torch.zeros(n, d, dtype=t, device=DEV)
+    v = (torch.linspace(-1, 2, n, device=DEV)[:, None] + torch.randn(n, d, device=DEV, generator=_gen(1)) * 0.1).to(t)
+    o = _attention_same_heads(q, k, v, heads, type, causal, 0.125)
+    count = torch.arange(1, n + 1, device=DEV, dtype=torch.float64)[:, None]
+    mean = v.double().cumsum(0) / count if causal else v.double().mean(0).expand(n, d)
+    mag = v.double().abs().cumsum(0) / count if causal else v.double().abs().mean(0).expand(n, d)
+    # the weights are all 1, exact in either type: what is left are f32 sums of n terms, and the result's rounding
+    u = mx_ref.half_step(t)
+    assert ((o.double() - mean).abs() <= (n + 2) * 2.0 ** -23 * mag + u * mean.abs() + 2.0 ** -25).all()
+
+
+@pytest.mark.parametrize("type", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("at", [0, 13, 63, 127, 128, 200, 255, 256, 300, 383, 400, 519])
+def test_attention_two_tiles_nan_keys(at, d, type):
+    """As test_attention_nan_keys_reach_the_rows_that_see_them, in CTAs of two tiles."""
+    n, t = 520, mx_ref.TYPES[type]
+    q, k, v = (torch.randn(n, d, device=DEV, generator=_gen(at + i)).to(t) for i in range(3))
+    k[at] = math.nan
+    assert torch.isnan(_attention_same_heads(q, k, v, 160, type, 0, d ** -0.5)).all()
+    o = _attention_same_heads(q, k, v, 160, type, 1, d ** -0.5)
+    assert torch.isnan(o[at:]).all() and torch.isfinite(o[:at]).all()
+
+
+@pytest.mark.parametrize("type", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n,gone", [(300, 30), (300, 128), (300, 200), (520, 384), (520, 130), (520, 520)])
+def test_attention_two_tiles_scores_of_minus_infinity(n, gone, d, type):
+    """As test_attention_scores_of_minus_infinity, in CTAs of two tiles."""
+    t = mx_ref.TYPES[type]
+    q, k, v = (torch.randn(n, d, device=DEV, generator=_gen(n + i)).to(t) for i in range(3))
+    q[:, 0] = 1.0
+    k[:gone, 0] = -math.inf
+    k[gone:, 0] = 0.0
+    for causal in (0, 1):
+        o = _attention_same_heads(q, k, v, 160, type, causal, d ** -0.5)
+        first = gone if causal or gone == n else 0
+        assert torch.isnan(o[:first]).all()
+        if first < n:
+            ref, mag = mx_ref.attention(q, k, v, [n], 1, 1, d, causal, d ** -0.5)
+            qk = d * 2.0 ** -23 * q.double().abs().amax() * k[gone:].double().abs().amax()
+            u = mx_ref.half_step(t)
+            tol = (1.01 * u + 1e-5 + 2 * qk) * mag + u * ref.abs()
+            if t == torch.float16:
+                tol = tol + n * 2.0 ** -36 * v.double().abs().amax() + 2.0 ** -25
+            assert ((o[first:].double() - ref[first:]).abs() <= tol[first:]).all()
+
+
+@pytest.mark.parametrize("heads", FEW_OR_MANY)
+@pytest.mark.parametrize("type", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_infinities_of_long_other_sequences(d, type, heads):
+    """A sequence full of NaN and infinities between two others, each of several tiles and key blocks."""
+    lens, t = [270, 400, 301], mx_ref.TYPES[type]
+    n = sum(lens)
+    clean = [torch.randn(n, d, device=DEV, generator=_gen(d + i)).to(t) for i in range(3)]
+    dirty = [x.clone() for x in clean]
+    for x in dirty:
+        x[270:670] = math.nan
+        x[270:670:2] = math.inf
+    keep = torch.cat([torch.arange(270), torch.arange(670, n)]).to(DEV)
+    for causal in (0, 1):
+        a, b = (_attention_same_heads(*x, heads, type, causal, d ** -0.5, lens) for x in (dirty, clean))
+        assert torch.equal(a[keep], b[keep]) and torch.isfinite(a[keep]).all()
+
+
+@pytest.mark.parametrize("heads", FEW_OR_MANY)
+@pytest.mark.parametrize("d", [64, 128])
+def test_attention_unseen_keys_of_several_tiles_weigh_nothing(d, heads):
+    """As test_attention_weight_of_unseen_keys_is_zero, over several key blocks: rows up to 300 see zeros only."""
+    n = 600
+    q, k = (torch.randn(n, d, device=DEV, generator=_gen(i)).bfloat16() for i in range(2))
+    v = torch.full((n, d), 2.0 ** 127, device=DEV).bfloat16()
+    v[:300] = 0.0
+    o = _attention_same_heads(q, k, v, heads, BF16, 1, d ** -0.5)
+    assert (o[:300] == 0).all()
+
+
+@pytest.mark.parametrize("heads", FEW_OR_MANY)
+@pytest.mark.parametrize("type", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("fall", [False, True])
+def test_attention_growing_scores_of_either_form(fall, d, type, heads):
+    """As test_attention_sharp_and_growing_scores, with the largest scores last or first, in both forms."""
+    t = mx_ref.TYPES[type]
+    n = 900
+    gain = torch.linspace(4, 0.1, n, device=DEV) if fall else torch.linspace(0.1, 4, n, device=DEV)
+    q, k, v = (torch.randn(n, d, device=DEV, generator=_gen(d + i)) for i in range(3))
+    q, k, v = q.to(t), (k * gain[:, None]).to(t), v.to(t)
+    for causal in (0, 1):
+        o = _attention_same_heads(q, k, v, heads, type, causal, d ** -0.5)
+        ref, mag = mx_ref.attention(q, k, v, [n], 1, 1, d, causal, d ** -0.5)
+        u = mx_ref.half_step(t)
+        tol = (1.01 * u + 4e-4) * mag + u * ref.abs() + (n * 2.0 ** -36 * 5 + 2.0 ** -25 if t == torch.float16 else 1e-30)
+        assert ((o.double() - ref).abs() <= tol).all()
+
+
 def test_attention_far_rows():
     """Token offsets that pass 32 bits."""
     n, ld, d = 66000, 33000 // 8 * 8, 64
