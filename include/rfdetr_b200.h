@@ -317,7 +317,9 @@ int rfdetr_b200_op_mx_dequantize(const void* codes, int ld_codes, const void* sc
 /* out[M][N] = act(A[M][K] . B[N][K]^T + bias) of two microscaled operands,
  * f32 accumulation, out of `out_type` with pitch ldo (elements).  bias f32 [N]
  * or NULL; act as rfdetr_b200_op_gemm (0 none, 1 GELU (erf), 2 ReLU, 3 SiLU),
- * NaN for NaN.  K at most 2^27. */
+ * NaN for NaN.  The sums are off by at most K 2^-29 of the sum of the products'
+ * magnitudes (the tensor core cuts them to f32); K at most 2^21, where that is
+ * half a step of BF16. */
 int rfdetr_b200_op_mx_gemm(const void* a, int lda, const void* a_scales, const void* b, int ldb, const void* b_scales,
                            int M, int N, int K, int act, const float* bias, void* out, int out_type, int ldo,
                            void* stream);
@@ -362,15 +364,17 @@ int rfdetr_b200_op_block_norm(const rfdetr_b200_block_norm* args, void* stream);
  * [tokens][kv_heads * head_dim], F16 or BF16, 16-byte aligned with pitches
  * that are multiples of 8; head h reads keys and values of head h / (heads /
  * kv_heads), at most 128 heads to one.  head_dim 64 or 128; max_len: at least
- * the longest length, and at most 2^25; 0 < scale <= 2e38, and scores
+ * the longest length, and at most 2^19; 0 < scale <= 2e38, and scores
  * (scale * q . k) of at most 2^26 in magnitude.  The lengths stay on the device.
- * Scores, their maximum and the sum of the weights are f32; each weight is
- * rounded to `type` for its product with v: off by at most 2^-8 (BF16) or
- * 2^-11 (F16) of itself or, in F16, 2^-36 of the row's largest, so a result by
- * that part of the weighted mean of |v| before its own rounding.  A row whose every score is -infinity is NaN.  A NaN query or
- * key reaches the rows that see it; an infinity or a NaN in v may also reach
- * rows of its sequence from which `causal` hides it (0 times infinity), as in
- * the plain form.  Neither reaches another sequence's rows. */
+ * Scores, their maximum and the sums are f32.  Each weight is rounded to `type`
+ * for its product with v: off by at most 2^-8 (BF16) or 2^-11 (F16) of itself
+ * or, in F16, 2^-36 of the row's largest; the tensor core cuts the sum of n
+ * products to f32: off by at most n 2^-27.  Both are parts of the weighted mean
+ * of |v|; then the result is rounded to `type`.
+ * A row whose every score is -infinity is NaN.  A NaN query or key reaches the
+ * rows that see it; an infinity or a NaN in v may also reach rows of its sequence
+ * from which `causal` hides it (0 times infinity), as in the plain form.  Neither
+ * reaches another sequence's rows. */
 int rfdetr_b200_op_attention_packed(const void* q, const void* k, const void* v, int ldq, int ldk, int ldv, void* o,
                                     int ldo, int type, const int32_t* cu_seqlens, int n_seqs, int tokens, int max_len,
                                     int heads, int kv_heads, int head_dim, int causal, float scale, void* stream);

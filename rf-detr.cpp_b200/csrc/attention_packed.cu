@@ -48,8 +48,8 @@ constexpr int TK = 128;               // keys of a block
 // most of it the result's own rounding); the sums below them are those of the f32 weights.  The
 // reference is a row's maximum less LIFT, and moves when the maximum grows by more than RAISE (both log2).  bf16 rounds a
 // weight by at most 2^-8 of it, however small.  f16 does so down to 2^-14 and holds less in steps of 2^-24: with the
-// reference 2^11 below the maximum a weight is off by at most 2^-36 of its row's largest, and 2^25 of them, the most that a
-// row has, together by half a step of f16.  (Without it by 2^-25 each: 65535 weights of 2^-25.2, 1.7e-3 of the row, were 0.)
+// reference 2^11 below the maximum a weight is off by at most 2^-36 of its row's largest, and 2^19 of them, the most that a
+// row has, together by 2^-17.  (Without it by 2^-25 each: 65535 weights of 2^-25.2, 1.7e-3 of the row, were 0.)
 // The largest weight is 2^(LIFT + RAISE) = 2^15; f16 ends at 2^16.
 template <typename T>
 struct Weights {
@@ -669,9 +669,11 @@ cudaError_t launch(const void* q, const void* k, const void* v, int ldq, int ldk
 cudaError_t attention_packed(const void* q, const void* k, const void* v, int ldq, int ldk, int ldv, void* o, int ldo,
                              int type, const int32_t* cu_seqlens, int n_seqs, int tokens, int max_len, int heads,
                              int kv_heads, int head_dim, int causal, float scale, cudaStream_t st) {
-    // max_len: an item ends well within the limit of the waits for it
+    // max_len: the tensor core cuts the f32 sums of P V, not rounds them, with every 16 keys: off by at most max_len 2^-27 of
+    // the weighted mean of |v|, toward 0.  Up to this length that is half a step of bf16 (equal weights, values of one sign:
+    // 1.7e-4 at 2^16, 1.4e-3 at 2^18, 6.5e-3 at 2^20; O in two parts would need the TMEM that the scores have).
     if ((type != MX_F16 && type != MX_BF16) || (head_dim != 64 && head_dim != 128) || n_seqs < 0 || tokens < 0 ||
-        max_len < 0 || max_len > (1 << 25) || heads < 1 || kv_heads < 1 || heads % kv_heads || heads / kv_heads > 128 ||
+        max_len < 0 || max_len > (1 << 19) || heads < 1 || kv_heads < 1 || heads % kv_heads || heads / kv_heads > 128 ||
         heads > INT32_MAX / 128 || !(scale > 0.f) || scale > 2e38f)  // scale / ln 2 is finite
         return cudaErrorInvalidValue;
     if (ldq < heads * head_dim || ldo < heads * head_dim || ldk < kv_heads * head_dim || ldv < kv_heads * head_dim ||

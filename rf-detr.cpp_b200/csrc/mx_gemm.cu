@@ -808,8 +808,10 @@ cudaError_t dispatch(const MxOperands& o, MxArgs p, cudaStream_t st) {
 cudaError_t mx_gemm(const uint8_t* a, int lda, const uint8_t* a_scales, const uint8_t* b, int ldb,
                     const uint8_t* b_scales, int M, int N, int K, int act, const float* bias, void* out, int out_type,
                     int ldo, cudaStream_t st) {
-    // K: a tile's products end well within the limit of the waits for them
-    if (M < 0 || N < 0 || K < 1 || K > (1 << 27) || M > INT32_MAX - 255 || N > INT32_MAX - 255 || ldo < N ||
+    // K: the tensor core cuts the f32 sum, not rounds it, with every 64 columns: off by at most K 2^-29 of the sum of the
+    // magnitudes, toward 0.  Up to this K that is half a step of bf16 (sums of one sign, scales far apart: 1.4e-5 at 2^16,
+    // split over a cluster 3.3e-5 at 2^20).
+    if (M < 0 || N < 0 || K < 1 || K > (1 << 21) || M > INT32_MAX - 255 || N > INT32_MAX - 255 || ldo < N ||
         !mx_type_ok(out_type) || act < ACT_NONE || act > ACT_SILU)
         return cudaErrorInvalidValue;
     if (M == 0 || N == 0) return cudaSuccess;

@@ -507,6 +507,26 @@ def test_gemm_one_block_of_each_row(M, N, K):
         assert torch.equal(out.double(), A @ B.T)
 
 
+@pytest.mark.parametrize("M,N,K", [(1, 40, 2 ** 21), (40, 64, 2 ** 18), (100, 64, 2 ** 18), (1200, 4096, 2 ** 14)])
+def test_gemm_long_sums_of_one_sign(M, N, K):
+    """Sums that only grow, of terms far apart: the tensor core cuts them with every 64 columns, by less than 2^-23."""
+    g = _gen(K)
+    ops = []
+    for rows in (M, N):
+        codes = torch.randint(0, 256, (rows, K // 2), device=DEV, generator=g).to(torch.uint8) & 0x77
+        ops.append((codes, torch.randint(122, 132, (rows, K // 32), device=DEV, generator=g).to(torch.uint8)))
+    (a, ea), (b, eb) = ops
+    out = torch.zeros(M, N, device=DEV)
+    assert _lib().rfdetr_b200_op_mx_gemm(_p(a), K // 2, _p(mx_ref.tile_scales(ea)), _p(b), K // 2, _p(mx_ref.tile_scales(eb)),
+                                         M, N, K, 0, None, _p(out), F32, N, _stream()) == 0
+    ref = torch.zeros(M, N, dtype=torch.float64, device=DEV)
+    for c in range(0, K, 2 ** 15):
+        A, B = (mx_ref.values(mx_ref.unpack(x[:, c // 2:c // 2 + 2 ** 14]), e[:, c // 32:c // 32 + 1024])[:, :K - c] for x, e in ops)
+        ref += A @ B.T
+    # then up to eight parts are added, and the result is an f32
+    assert ((out.double() - ref).abs() <= (K * 2.0 ** -29 + 9 * 2.0 ** -24) * ref).all()
+
+
 @pytest.mark.parametrize("M,N,K", [(2400, 2051, 600), (2400, 2051, 2050)])
 def test_gemm_wide_tiles_are_deterministic(M, N, K):
     first = _gemm(M, N, K, 1, F32, True)
@@ -946,6 +966,21 @@ def test_attention_weight_of_unseen_keys_is_zero(d):
     v[0] = 0.0
     o = _attention_once(q, k, v, d, BF16, 1, d ** -0.5)
     assert (o[0] == 0).all()
+
+
+@pytest.mark.parametrize("type", [F16, BF16])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("n", [2 ** 16, 2 ** 18 + 1, 2 ** 19])
+def test_attention_long_sums_of_one_sign(n, d, type):
+    """Equal weights and values of one sign: the tensor core cuts its sums with every 16 keys, by less than 2^-23."""
+    t = mx_ref.TYPES[type]
+    q, k = torch.zeros(n, d, dtype=t, device=DEV), torch.zeros(n, d, dtype=t, device=DEV)
+    v = (1 + torch.rand(n, d, device=DEV, generator=_gen(n))).to(t)
+    o = _attention_once(q, k, v, d, type, 0, 1.0)
+    ref = v.double().mean(0)
+    # the sum of the weights is one of n / 128 terms a row, of 32 each
+    u = mx_ref.half_step(t)
+    assert ((o.double() - ref).abs() <= (n * 2.0 ** -27 + (n / 128 + 40) * 2.0 ** -24 + 1e-6 + u) * ref).all()
 
 
 # Heads of one sequence that a B200's 148 SMs take as single tiles whose keys are shared out, and so many that a CTA has
