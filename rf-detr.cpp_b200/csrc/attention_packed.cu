@@ -606,6 +606,7 @@ k_attn_packed(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ C
             }
         }
     }
+    linger_if_aborted(cta_abort);
     tc_fence_before();
     __syncthreads();
     report_abort(cta_abort, p.err);

@@ -447,6 +447,7 @@ k_mx_gemm(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUten
         }
         if (p.tma_out && elect_one()) bulk_wait<0>();
     }
+    linger_if_aborted(cta_abort);
     tc_fence_before();
     if constexpr (CTA2) cluster_sync();  // the peer may still arrive here, and the pair frees its TMEM together
     else __syncthreads();
@@ -660,8 +661,12 @@ k_mx_gemm_few(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ C
             }
         }
     }
+    linger_if_aborted(cta_abort);
     __syncwarp();
-    if (parts > 1) cluster_sync();  // nobody still reads or writes another's shared memory
+    if (parts > 1) {
+        cluster_sync();  // nobody still reads or writes another's shared memory,
+        linger_if_aborted(cta_abort);  // but for what was sent to a CTA that no longer waits for it
+    }
     tc_fence_before();
     __syncthreads();
     report_abort(cta_abort, p.err);

@@ -113,6 +113,16 @@ __device__ __forceinline__ void report_abort(const volatile int* cta_abort, int*
     if (threadIdx.x == 0 && *cta_abort) atomicCAS(err, 0, kErrWaitTimeout);
 }
 
+// Before a CTA's last barrier, and behind its cluster's: where a wait ran out, copies and products may be in flight that no
+// wait covers any more.  They take microseconds; they get 10 ms before the CTA frees its tensor memory and leaves (a thread
+// that saw a wait run out sees the word, and the barrier waits for it).
+constexpr unsigned long long kLingerNs = 10000000ull;
+__device__ __forceinline__ void linger_if_aborted(const volatile int* cta_abort) {
+    if (!*cta_abort) return;
+    const unsigned long long t0 = globaltimer();
+    while (globaltimer() - t0 < kLingerNs) {}
+}
+
 // 3-D tiled TMA load global -> shared, completing on `bar` (complete_tx).
 __device__ __forceinline__ void tma_load_3d(const CUtensorMap* map, uint64_t* bar, void* dst, int x, int y, int z) {
     asm volatile(

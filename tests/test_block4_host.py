@@ -181,3 +181,15 @@ def test_sums_too_long_for_f32_are_refused():
     assert L.rfdetr_b200_op_mx_gemm(P, 2 ** 21, P, P, 2 ** 21, P, 1, 1, k, 0, None, P, 0, 1, None) == INVALID
     assert L.rfdetr_b200_op_attention_packed(P, P, P, 64, 64, 64, P, 64, 1, P, 1, 2 ** 20, 2 ** 19 + 1, 1, 1, 64, 0, 0.125,
                                              None) == INVALID
+
+
+@pytest.mark.parametrize("name,kernel,before", [
+    ("mx_gemm.cu", "k_mx_gemm", r"tc_fence_before\(\);\s*if constexpr \(CTA2\) cluster_sync\(\);\s*else __syncthreads\(\);"),
+    ("mx_gemm.cu", "k_mx_gemm_few", r"__syncwarp\(\);\s*if \(parts > 1\) \{\s*cluster_sync\(\);\s*linger_if_aborted\(cta_abort\);"),
+    ("attention_packed.cu", "k_attn_packed", r"tc_fence_before\(\);\s*__syncthreads\(\);")])
+def test_a_cta_that_gives_up_waits_for_what_is_in_flight(name, kernel, before):
+    """Behind the roles, in front of the barrier that ends in freeing tensor memory and leaving (and behind the
+    cluster's, where others send to this CTA)."""
+    code = _kernel(name, kernel)
+    at = re.search(r"linger_if_aborted\(cta_abort\);\s*" + before, code)
+    assert at and code.rindex("mbar_wait") < at.start() < code.index("report_abort") < code.index("tmem_dealloc")
