@@ -1272,6 +1272,71 @@ def test_block_together(type):
     assert ((b["hid"].double() - ref).abs() <= _gemm_tolerance(A, b["f_v"], ref, t, 3, None)).all()
 
 
+@pytest.mark.parametrize("type", [F16, BF16])
+def test_block_to_its_end(type):
+    """The block's second half behind the hidden layer: quantisation, the product back to the residual stream's width,
+    norm and residual, and the next block's norm with its operand; directly and captured."""
+    from rfdetr_b200 import lib
+
+    c = CONFIG
+    n, dim, hidden = sum(c["lens"]), c["dim"], c["hidden"]
+    t, L = mx_ref.TYPES[type], _lib()
+    b = _block_buffers(type, seed=5, **c)
+    g = _gen(6)
+    w, sw, W = _operand(g, dim, hidden)
+    sw, W = (sw.int() - 4).clamp_min(0).to(torch.uint8), W / 16
+    w4, w5 = (1 + 0.1 * torch.randn(dim, device=DEV, generator=g) for _ in range(2))
+
+    def run(stream, hc, hs, z, x2, h, nc, ns):
+        _block(type, bufs=b, L=L, lib=lib, stream=stream, **c)
+        rc = [L.rfdetr_b200_op_mx_quantize(_p(b["hid"]), type, hidden, n, hidden, _p(hc), hidden // 2, _p(hs), stream)]
+        rc.append(L.rfdetr_b200_op_mx_gemm(_p(hc), hidden // 2, _p(hs), _p(w), hidden // 2, _p(sw), n, dim, hidden, 0, None,
+                                           _p(z), type, dim, stream))
+        rc.append(L.rfdetr_b200_op_block_norm(lib.BlockNorm(
+            y=_p(z), resid=_p(b["x1"]), post=2, post_w=_p(w4), out_resid=_p(x2), pre=2, pre_w=_p(w5), out=_p(h),
+            mx_codes=_p(nc), mx_scales=_p(ns), rows=n, dim=dim, type=type, resid_type=F32, ldy=dim, ld_resid=dim,
+            ld_out_resid=dim, ld_out=dim, ld_mx=dim // 2, resid_scale=1.0, post_eps=1e-6, pre_eps=1e-6), stream))
+        assert rc == [0] * 3
+
+    def buffers():
+        return [*_mx_buffers(n, hidden), torch.zeros(n, dim, dtype=t, device=DEV), torch.zeros(n, dim, device=DEV),
+                torch.zeros(n, dim, dtype=t, device=DEV), *_mx_buffers(n, dim)]
+
+    out = buffers()
+    run(_stream(), *out)
+    hc, hs, z, x2, h, nc, ns = out
+    codes, e = mx_ref.quantize(b["hid"].double())
+    assert torch.equal(hc, mx_ref.pack(codes)) and torch.equal(hs, mx_ref.tile_scales(e))
+    A = mx_ref.values(codes, e)
+    ref = A @ W.T
+    assert ((z.double() - ref).abs() <= _gemm_tolerance(A, W, ref, t, 0, None)).all()
+    post, _ = mx_ref.norm(z.double(), 2, w4, None, 1e-6)
+    want = b["x1"].double() + post
+    # the sums' roundings are under 110 * 2^-24 (as in _norm_case), of the norms and of what they are added to
+    u = 110 * 2.0 ** -24
+    slack = u * (post.abs() + want.abs()) + 4 * 2.0 ** -24 * (post.abs() + b["x1"].double().abs())
+    assert ((x2.double() - want).abs() <= slack).all()
+    nxt, rstd = mx_ref.norm(want, 2, w5, None, 1e-6)
+    worst = slack.amax(1, keepdim=True) * rstd
+    tol = worst * (3 * w5.double().abs() + 2 * nxt.abs()) + u * nxt.abs() + mx_ref.half_step(t) * nxt.abs() + 2.0 ** -25
+    assert ((h.double() - nxt).abs() <= tol).all()
+    e = ns.view(-1, dim // 128, 32, 4, 4).permute(0, 3, 2, 1, 4).reshape(-1, dim // 32)[:n]
+    # E2M1's own steps: at most a sixth of a value in [1, 6] scales, a quarter scale below; 6 stands for up to 8
+    v, scale = mx_ref.values(mx_ref.unpack(nc), e), mx_ref.pow2(e.long() - 127).repeat_interleave(32, 1)
+    assert ((v - nxt).abs() <= torch.maximum(0.25 * scale, nxt.abs() / 4) + tol).all()
+
+    caught = buffers()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        run(torch.cuda.current_stream().cuda_stream, *caught)
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    for x, y in zip(caught, out):
+        assert torch.equal(x, y)
+
+
 def test_block_captured_and_replayed():
     """The same calls captured into a CUDA graph on a stream of their own and replayed on new inputs
     give what direct calls give, also while direct calls run on another stream."""
