@@ -316,10 +316,11 @@ int rfdetr_b200_op_mx_dequantize(const void* codes, int ld_codes, const void* sc
 
 /* out[M][N] = act(A[M][K] . B[N][K]^T + bias) of two microscaled operands,
  * f32 accumulation, out of `out_type` with pitch ldo (elements).  bias f32 [N]
- * or NULL; act as rfdetr_b200_op_gemm (0 none, 1 GELU (erf), 2 ReLU, 3 SiLU),
- * NaN for NaN.  The sums are off by at most K 2^-29 of the sum of the products'
- * magnitudes (the tensor core cuts them to f32); K at most 2^21, where that is
- * half a step of BF16. */
+ * or NULL; act as rfdetr_b200_op_gemm (0 none, 1 GELU (erf), 2 ReLU, 3 SiLU;
+ * NaN for NaN; GELU within 3.2e-7, SiLU within 2^-17 of itself and 0 below -87).
+ * The sums are off by at most K 2^-29 of the sum of the products' magnitudes
+ * (the tensor core cuts them to f32); K at most 2^21, where that is half a step
+ * of BF16.  out overlaps none of the operands. */
 int rfdetr_b200_op_mx_gemm(const void* a, int lda, const void* a_scales, const void* b, int ldb, const void* b_scales,
                            int M, int N, int K, int act, const float* bias, void* out, int out_type, int ldo,
                            void* stream);
@@ -362,7 +363,7 @@ int rfdetr_b200_op_block_norm(const rfdetr_b200_block_norm* args, void* stream);
  * written), O = softmax(scale * Q K^T) V within each, with `causal` up to the
  * query's own position.  q, o [tokens][heads * head_dim], k, v
  * [tokens][kv_heads * head_dim], F16 or BF16, 16-byte aligned with pitches
- * that are multiples of 8; head h reads keys and values of head h / (heads /
+ * that are multiples of 8, o apart from the others; head h reads keys and values of head h / (heads /
  * kv_heads), at most 128 heads to one.  head_dim 64 or 128; max_len: at least
  * the longest length, and at most 2^19; 0 < scale <= 2e38, and scores
  * (scale * q . k) of at most 2^26 in magnitude.  The lengths stay on the device.

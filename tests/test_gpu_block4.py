@@ -507,6 +507,32 @@ def test_gemm_one_block_of_each_row(M, N, K):
         assert torch.equal(out.double(), A @ B.T)
 
 
+@pytest.mark.parametrize("M", [1, 20, 260])
+@pytest.mark.parametrize("act", [0, 1, 2, 3])
+def test_gemm_activations_over_their_range(act, M):
+    """act(bias) alone, operands of zeros: GELU is within 3.2e-7 and f32's rounding; SiLU within 2^-17 of itself, the
+    fast exponential's 2 + 1.173 |v| steps and the quotient's 2, down to -87, and 0 below; the others are exact."""
+    K, N = 64, 4096
+    v = torch.cat([torch.linspace(-100, 100, N - 1000), torch.linspace(-8, 8, 990),
+                   torch.tensor([0.0, -0.0, 1e-30, -1e-30, 3e38, -3e38, math.inf, 88.0, -86.9, -120.0])]).to(DEV)
+    a, b = (torch.zeros(r, K // 2, dtype=torch.uint8, device=DEV) for r in (M, N))
+    sa, sb = (torch.zeros(_lib().rfdetr_b200_mx_scale_bytes(r, K), dtype=torch.uint8, device=DEV) for r in (M, N))
+    out = torch.full((M, N), 7.0, device=DEV)
+    assert _lib().rfdetr_b200_op_mx_gemm(_p(a), K // 2, _p(sa), _p(b), K // 2, _p(sb), M, N, K, act, _p(v), _p(out), F32, N,
+                                         _stream()) == 0
+    x = v.double()
+    if act in (0, 2):
+        want = v if act == 0 else v.clamp_min(0)
+        assert (out == want).all()
+        return
+    want = mx_ref.act(x, act)
+    want[torch.isposinf(v)] = math.inf
+    tol = 3.2e-7 + 2.0 ** -24 * x.abs() if act == 1 else torch.where(x > -87, 2.0 ** -17 * want.abs(), 1e-36)
+    fine = torch.isfinite(want)
+    assert ((out.double() - want).abs() <= tol)[:, fine].all()
+    assert (out[:, ~fine].double() == want[~fine]).all()
+
+
 @pytest.mark.parametrize("M,N,K", [(1, 40, 2 ** 21), (40, 64, 2 ** 18), (100, 64, 2 ** 18), (1200, 4096, 2 ** 14)])
 def test_gemm_long_sums_of_one_sign(M, N, K):
     """Sums that only grow, of terms far apart: the tensor core cuts them with every 64 columns, by less than 2^-23."""
