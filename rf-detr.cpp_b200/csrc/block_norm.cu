@@ -10,8 +10,9 @@
 // thread holds chunks of four columns (one 8- or 16-byte access of every operand, so a warp's accesses
 // of either type are without gaps), C of them.  Rows of up to 512 columns belong to one warp each,
 // longer ones to a CTA.  51712 x 384 f16 with an f32 residual: 37.5 us, 6.3 TB/s; 16 Mi elements of bf16 in and out:
-// 25.7 us (5.2 TB/s) in rows of 1024, 27.0 of 2048, 28.5 of 4096, 31.8 of 8192, where the instructions of the
-// 16-bit conversions and the two sums' barriers show.
+// 25.7 us (5.2 TB/s) in rows of 1024, 27.0 of 2048, 26-28.5 of 4096, 31-32 of 8192, where the two sums' barriers
+// show: one row's loads are in flight in a CTA.  Beyond, 1024 threads of 64 registers, some of which spill: 37 of
+// 16384, 42 of 32768, 71 of 20000, which end inside the threads' chunks.
 #include "mx.cuh"
 
 namespace rfb {
